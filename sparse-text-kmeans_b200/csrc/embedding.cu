@@ -739,9 +739,10 @@ int launch_grad(GradArgs& a, void* workspace, cudaStream_t st) {
 
 template <class TI, class TO>
 int pick_grad(GradArgs& a, void* ws, cudaStream_t st) {
-    // E elements: up to 16 bytes of either type at once, both sides aligned to that, and a divisor of the row
+    // E elements, a divisor of the row: up to 16 bytes of `grad` by one load and all of them to `out` by one store, which for eight
+    // sums of fp32 is one of 32 bytes; either side's rows start at multiples of the access
     auto fits = [&](uint32_t e) {
-        const uint64_t in = e * sizeof(TI) < 16 ? e * sizeof(TI) : 16, out = e * sizeof(TO) < 16 ? e * sizeof(TO) : 16;
+        const uint64_t in = e * sizeof(TI) < 16 ? e * sizeof(TI) : 16, out = e * sizeof(TO);
         Alignment i, o;
         i.add(a.grad).add(a.grad_stride * sizeof(TI));
         o.add(a.out).add(a.out_stride * sizeof(TO));

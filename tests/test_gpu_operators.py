@@ -166,6 +166,31 @@ def test_grad(cp, torch, types, n, rows, dim, kind, layout):
     assert torch.equal(room[idle], before[idle])
 
 
+@pytest.mark.parametrize("types", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("n,dim", [(300, 64), (2048, 1024), (2049, 64), (9000, 1024)])
+@pytest.mark.parametrize("first,more", [(0, 4), (4, 4), (4, 0), (4, 8), (2, 2), (8, 8)])
+def test_grad_into_part_of_a_buffer(cp, torch, types, n, dim, first, more):
+    """Rows of the output that start at any multiple of 4 to 32 bytes and at any distance: a slice of a flat buffer, columns of a
+    wider one.  Whole numbers: the sums are exact, and what lies beside them stays."""
+    gen = generator(torch, n + dim + 10 * first + more)
+    rows = 150
+    ids = ids_of(torch, gen, "zipf", n, rows)  # (the commonest id has more places than a piece)
+    grad = torch.randint(-2, 3, (n, dim), generator=gen, device="cuda").to(dtype_of(torch, types[0]))
+    want = grad_want(torch, ids, grad, rows, 0.5)[0]
+    want = want.to(dtype_of(torch, types[1]))  # (one rounding of an exact sum)
+    width = dim + more
+    for accumulate in (False, True):
+        flat = torch.full((first + rows * width + 40,), 1.0, dtype=want.dtype, device="cuda")
+        out = flat[first:first + rows * width].view(rows, width)[:, :dim]
+        assert cp.embedding_grad(ids, grad, rows, 0.5, out=out, accumulate=accumulate) is out
+        expect = torch.ones_like(flat)
+        inside = expect[first:first + rows * width].view(rows, width)[:, :dim]
+        # (with what was there: the sum in fp32 is exact too, and rounded once)
+        inside.copy_((grad_want(torch, ids, grad, rows, 0.5)[0] + 1.0).to(want.dtype) if accumulate else want)
+        assert torch.equal(flat, expect)
+    cp.check_operator_status()
+
+
 @pytest.mark.parametrize("n,rows,dim", [(1_100_007, 5000, 4), (2_200_000, 300, 3)])
 def test_grad_of_many_places(cp, torch, n, rows, dim):
     gen = generator(torch, n)
