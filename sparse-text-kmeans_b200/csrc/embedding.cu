@@ -793,7 +793,9 @@ int cphnsw_b200_embedding_lookup_dev(const void* d_table, int type, uint64_t row
 }
 
 uint64_t cphnsw_b200_embedding_grad_workspace(uint64_t n, uint64_t rows, uint64_t dim) {
-    return n <= kSmallMost ? 0 : GradSpace(n, rows, dim).bytes;
+    // (what the call refuses needs none; the digits of `rows` are counted by shifts of it)
+    if (n <= kSmallMost || n >= (1ull << 31) || rows >= (1ull << 31) || dim >= (1ull << 20)) return 0;
+    return GradSpace(n, rows, dim).bytes;
 }
 
 int cphnsw_b200_embedding_grad_dev(const void* d_ids, uint32_t id_bytes, uint64_t n, const void* d_grad, int grad_type,

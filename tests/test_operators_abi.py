@@ -1,5 +1,7 @@
 """The operators' C entry points refuse wrong arguments before they look for a device, and a machine without one."""
 import ctypes as C
+import subprocess
+import sys
 
 import pytest
 
@@ -90,3 +92,17 @@ def test_workspaces(lib):
     # rows of 100 bytes are copied to rows of 112, 256 bytes at a time
     assert lib.cphnsw_b200_int8_matmul_workspace(p(A), U(100), U(8), p(A), U(112), U(8), U(100)) == 1024
     assert lib.cphnsw_b200_distill_workspace(U(10), U(64)) >= 10 * 64 * 12
+
+
+def test_workspaces_of_refused_sizes(cp):
+    """Sizes that the calls refuse are answered too, and at once (a process of its own: one that does not answer is ended)."""
+    code = """
+import ctypes as C, sys
+fn = C.CDLL(sys.argv[1]).cphnsw_b200_embedding_grad_workspace
+fn.restype = C.c_uint64
+for n, rows, dim in [(5000, 2**64 - 1, 8), (5000, 2**63, 8), (5000, 2**31, 8), (2**31, 100, 8), (2**64 - 1, 100, 8), (5000, 100, 2**20)]:
+    assert fn(C.c_uint64(n), C.c_uint64(rows), C.c_uint64(dim)) == 0, (n, rows, dim)
+assert fn(C.c_uint64(5000), C.c_uint64(2**31 - 1), C.c_uint64(8)) > 2**31 * 4
+"""
+    done = subprocess.run([sys.executable, "-c", code, cp.LIB_PATH], timeout=60, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
