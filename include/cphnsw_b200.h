@@ -453,7 +453,8 @@ int cphnsw_b200_embedding_lookup_dev(const void* d_table, int type, uint64_t row
 
 /* out[v] = scale * sum over all i with ids[i] = v of grad[i]: the lookup's gradient, [rows][dim], of type fp32 or grad's.
  * accumulate != 0: it is added to what out holds, and rows that no id names are left alone.  Sums are fp32, rounded once, in
- * an order that depends on the ids alone: the same input gives the same bits.  n < 2^31. */
+ * an order that depends on the ids, dim and grad_type alone: the same input gives the same bits, whatever its strides.
+ * n < 2^31. */
 uint64_t cphnsw_b200_embedding_grad_workspace(uint64_t n, uint64_t rows, uint64_t dim);
 int cphnsw_b200_embedding_grad_dev(const void* d_ids, uint32_t id_bytes, uint64_t n, const void* d_grad, int grad_type,
                                    uint64_t grad_stride, float scale, void* d_out, int out_type, uint64_t rows, uint64_t dim,

@@ -191,6 +191,22 @@ def test_grad_into_part_of_a_buffer(cp, torch, types, n, dim, first, more):
     cp.check_operator_status()
 
 
+@pytest.mark.parametrize("name", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,rows,dim", [(300, 15, 512), (300, 15, 300), (2048, 40, 96), (1000, 5, 1024), (2000, 3, 255), (5000, 200, 512), (5000, 3, 96)])
+def test_grad_bits_of_other_layouts(cp, torch, name, n, rows, dim):
+    """The order of a sum does not depend on where rows start: the same bits from, and to, every layout."""
+    gen = generator(torch, n + dim)
+    ids = ids_of(torch, gen, "even", n, rows)
+    grad = torch.randn((n, dim), generator=gen, device="cuda").to(dtype_of(torch, name))
+    for dtype in {torch.float32, grad.dtype}:
+        want = cp.embedding_grad(ids, grad, rows, 1.75, dtype=dtype)
+        for layout in ("padded", "shifted"):
+            assert torch.equal(cp.embedding_grad(ids, laid_out(torch, grad, layout), rows, 1.75, dtype=dtype), want)
+        for first, more in ((0, 1), (1, 8), (2, 6), (4, 4), (4, 8), (8, 8)):
+            room = torch.zeros((rows, first + dim + more), dtype=dtype, device="cuda")
+            assert torch.equal(cp.embedding_grad(ids, grad, rows, 1.75, out=room[:, first:first + dim]), want)
+
+
 @pytest.mark.parametrize("n,rows,dim", [(1_100_007, 5000, 4), (2_200_000, 300, 3)])
 def test_grad_of_many_places(cp, torch, n, rows, dim):
     gen = generator(torch, n)
