@@ -885,45 +885,6 @@ int launch_loss(const Args& a, uint64_t words, cudaStream_t st) {
         default: return launch_clusters(distill_loss_kernel<T, 512>, 512, a, a.n * cluster, cluster, bytes, st);
     }
 }
-// Clusters of a kernel that run at once, asked for once per device and launch shape
-template <class K>
-int clusters_at_once(K* kernel, int threads, uint32_t cluster, uint32_t smem, uint64_t* out) {
-    struct Known {
-        const void* kernel;
-        int device;
-        uint32_t cluster, smem;
-        int many;
-    };
-    static std::mutex mutex;
-    static Known known[64];
-    static int used = 0;
-    int dev = 0;
-    CPB_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lock(mutex);
-    for (int i = 0; i < used && i < 64; ++i)
-        if (known[i].kernel == reinterpret_cast<const void*>(kernel) && known[i].device == dev && known[i].cluster == cluster && known[i].smem == smem) {
-            *out = known[i].many;
-            return 0;
-        }
-    CPB_CUDA(allow_max_dynamic_smem(kernel));
-    if (cluster > 8) CPB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int many = 0;
-    CPB_CUDA(cudaOccupancyMaxActiveClusters(&many, kernel, &cfg));
-    if (many < 1) many = 1;
-    known[used++ % 64] = {reinterpret_cast<const void*>(kernel), dev, cluster, smem, many};
-    *out = many;
-    return 0;
-}
 template <class T, int kHeld>
 int launch_short(const Args& a, uint32_t smem, cudaStream_t st) {
     auto kernel = distill_short_kernel<T, kHeld>;
@@ -932,10 +893,12 @@ int launch_short(const Args& a, uint32_t smem, cudaStream_t st) {
     CPB_CUDA(cudaGetLastError());
     return 0;
 }
+// shared memory of a block, at most: what lists leave goes to the ring
+constexpr uint32_t ring_bytes(int warps) { return kRingBytes / ring_blocks(warps) - (ring_blocks(warps) - 1) * 4096; }
 // places of a ring, beside the lists
 template <int kWarps>
 uint32_t ring_slots(uint32_t top) {
-    const uint32_t bytes = kRingBytes / ring_blocks(kWarps) - (ring_blocks(kWarps) - 1) * 4096, lists = kAhead * list_bytes(top);
+    const uint32_t bytes = ring_bytes(kWarps), lists = kAhead * list_bytes(top);
     const uint32_t slots = bytes > lists ? (bytes - lists) / kChunkBytes : 0;
     return slots < kMaxSlots ? slots : kMaxSlots;
 }
@@ -947,6 +910,39 @@ uint64_t ring_share(uint32_t top) {
     const uint32_t slots = ring_slots<kWarps>(top);
     return slots <= kWarps ? 0 : uint64_t(slots + kWarps) / 2 * kChunkWords;
 }
+// Clusters of the ring's kernel that run at once, asked for once per device and size of cluster.  The length of the lists does not
+// come into it: a ring takes what they leave but for less than a place, or 52 places, so that an SM has room for ring_blocks blocks
+// and no more whatever the length.  (Asked for again with every length, eleven sizes took the host 4.7 us of 21 a call.)
+template <class T, bool GIVEN, int kWarps>
+int clusters_at_once(uint32_t cluster, uint64_t* out) {
+    static_assert(ring_blocks(kWarps) * ring_bytes(kWarps) < 227 * 1024 && (ring_blocks(kWarps) + 1) * (ring_bytes(kWarps) - kChunkBytes) > 227 * 1024 &&
+                      (ring_bytes(kWarps) < kMaxSlots * kChunkBytes || (ring_blocks(kWarps) + 1) * kMaxSlots * kChunkBytes > 227 * 1024),
+                  "blocks an SM");
+    static std::atomic<int> known[op::kMaxDevices][kMaxRing + 1];
+    int dev = 0;
+    CPB_CUDA(cudaGetDevice(&dev));
+    int many = known[dev][cluster].load(std::memory_order_relaxed);
+    if (!many) {
+        auto kernel = distill_ring_kernel<T, GIVEN, kWarps>;
+        CPB_CUDA(allow_max_dynamic_smem(kernel));
+        if (cluster > 8) CPB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(cluster);
+        cfg.blockDim = dim3(ring_threads(kWarps));
+        cfg.dynamicSmemBytes = ring_bytes(kWarps);
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = cluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        CPB_CUDA(cudaOccupancyMaxActiveClusters(&many, kernel, &cfg));
+        if (many < 1) many = 1;
+        known[dev][cluster].store(many, std::memory_order_relaxed);
+    }
+    *out = many;
+    return 0;
+}
 template <class T, bool GIVEN, int kWarps>
 int launch_ring(Args& a, uint64_t words, uint32_t parts, cudaStream_t st) {
     a.slots = ring_slots<kWarps>(a.top);
@@ -954,7 +950,7 @@ int launch_ring(Args& a, uint64_t words, uint32_t parts, cudaStream_t st) {
     auto kernel = distill_ring_kernel<T, GIVEN, kWarps>;
     uint64_t most = 0;
     if (GIVEN) {
-        CPB_TRY(clusters_at_once(kernel, ring_threads(kWarps), 1, smem, &most));
+        CPB_TRY((clusters_at_once<T, GIVEN, kWarps>(1, &most)));
     } else {
         // More blocks a row than it takes, where clusters of that size leave SMs over that larger ones do not (their SMs have to
         // lie together): 1,000 rows of 700,001 bf16 logits, 11 blocks a row 784 us, 16 549.  3, 5, 6 and 7 are left out: as many
@@ -965,7 +961,7 @@ int launch_ring(Args& a, uint64_t words, uint32_t parts, cudaStream_t st) {
         for (uint32_t size = parts; size <= (parts == 1 ? 1 : kMaxRing); ++size) {
             if (size < 8 && (size & (size - 1)) != 0) continue;
             uint64_t many = 0;
-            CPB_TRY(clusters_at_once(kernel, ring_threads(kWarps), size, smem, &many));
+            CPB_TRY((clusters_at_once<T, GIVEN, kWarps>(size, &many)));
             if (many * size * 32 > used * 33) used = many * size, best = size, most = many;
         }
         parts = best;

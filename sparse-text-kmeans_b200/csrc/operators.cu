@@ -5,7 +5,6 @@ namespace cpb {
 namespace op {
 namespace {
 
-constexpr int kMaxDevices = 64;
 __device__ uint32_t g_operator_status;
 std::mutex g_mutex;
 uint32_t* g_status_ptr[kMaxDevices] = {};

@@ -147,8 +147,9 @@ struct Alignment {
 // The word that bounded waits of the operators' kernels raise, one per device
 int status_word(uint32_t** out);
 
+constexpr int kMaxDevices = 64;
 int sm_count(int* out);  // of the current device
-int check_device();  // the current device is one this library runs on
+int check_device();  // the current device is one this library runs on, its number below kMaxDevices
 inline int invalid(const char* what) {
     set_error("%s", what);
     return CPHNSW_B200_E_INVALID;

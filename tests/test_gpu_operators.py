@@ -5,6 +5,7 @@ Tolerances follow from the arithmetic, before any run: u is half a unit in the l
 of the sum of magnitudes.  Results of fp16 below its normal numbers are allowed half their spacing, 2^-25.
 """
 import math
+import time
 
 import pytest
 
@@ -460,6 +461,28 @@ def test_distill_grad_against_differences(cp, torch, rows):
     # a loss is off by at most 2^-16 T^2 (1 + 2^-4 * 20); the third derivative along a direction of length 1 is below 2 / T
     bound = 2 * T * T * 2.0 ** -16 * 2.25 / (2 * h) + h * h / 6 * 2 / T + 2.0 ** -15
     assert float(((up - down) / (2 * h) - (grad.double() * d.double()).sum(1)).abs().max()) <= bound
+
+
+def test_distill_lists_of_many_lengths(cp, torch):
+    """What a launch asks of the driver it asks once, not again with every length of the lists: the host takes as long for calls
+    of forty lengths in turn as for forty of one.  Eleven questions take 4 us and more; 2 us a call are allowed."""
+    n, rows, calls = 40, 100_003, 40
+    z = torch.randn((n, rows), device="cuda").bfloat16()
+    out = torch.empty_like(z)
+    ids = torch.randint(0, rows, (n, calls), device="cuda")
+    teacher = torch.randn((n, calls), device="cuda")
+    lists = [(ids[:, :top].contiguous(), teacher[:, :top].contiguous()) for top in range(1, calls + 1)]
+
+    def host(lists):
+        torch.cuda.synchronize()
+        start = time.perf_counter()
+        for i, t in lists:
+            cp.distill_loss_and_grad(z, i, t, out=out)
+        return (time.perf_counter() - start) / calls * 1e6
+
+    turns = [(host([lists[9]] * calls), host(lists)) for _ in range(30)][1:]  # (the shortest of each: the host does other things too)
+    one, many = (min(t[k] for t in turns) for k in range(2))
+    assert many <= one + 2.0, (many, one)
 
 
 # ---- the whole, other streams, refusals --------------------------------------------------------------------------------------
