@@ -7,10 +7,12 @@ of 8-bit vectors (``quantize_rows``, ``int8_matmul``), which score queries again
 
 Every call runs on the current torch stream of its tensors' device, returns without waiting, and takes its outputs and its
 workspace from torch's allocator; a tensor that another stream has written or will reuse is the caller's to synchronise, as
-with torch's own operations.  No autograd graph is recorded: the gradients are calls of their own.  Matrices may have any row
-stride (0 for a broadcast row); where the elements of a row are not next to one another a contiguous copy is made.  Wrong
-arguments raise ``ValueError`` before anything is launched.  ``check_operator_status`` waits for the device and raises if a
-kernel gave up a bounded wait.
+with torch's own operations.  No autograd graph is recorded: the gradients are calls of their own.  While gradients are
+recorded a tensor that requires one is therefore refused (``detach()`` it, or call under ``torch.no_grad()``), except as
+the logits of ``distill_loss_and_grad``, whose gradient that call returns (``logits.backward(grad)`` goes on from
+there).  Matrices may have any row stride (0 for a broadcast row); where the elements of a row are not next to one
+another a contiguous copy is made.  Wrong arguments raise ``ValueError`` before anything is launched.
+``check_operator_status`` waits for the device and raises if a kernel gave up a bounded wait.
 """
 import ctypes as C
 
@@ -53,8 +55,8 @@ def _bind():
     _torch = torch
 
 
-def _device(*tensors):
-    """The index of the tensors' one device."""
+def _device(*tensors, differentiable=None):
+    """The index of the tensors' one device.  What the caller would lose a gradient of is refused, but for ``differentiable``."""
     if _torch is None:
         _bind()
     dev = None
@@ -66,6 +68,8 @@ def _device(*tensors):
             dev = at
         elif at != dev:
             raise ValueError("tensors on several devices")
+        if t.requires_grad and t is not differentiable and _torch.is_grad_enabled():
+            raise ValueError("a tensor that requires a gradient: no graph is recorded here; pass t.detach(), or call under torch.no_grad()")
     return dev
 
 
@@ -243,7 +247,8 @@ def distill_loss(logits, ids, teacher, temperature=1.0):
 def distill_loss_and_grad(logits, ids, teacher, weight=None, temperature=1.0, out=None):
     """``distill_loss`` and the gradient of its sum, weighted by ``weight`` float32 [n] (1 unless given), with respect to the
     logits, in their type: (loss [n], grad [n, rows]).  ``out`` may be ``logits`` itself."""
-    dev = _device(logits, ids, teacher) if weight is None else _device(logits, ids, teacher, weight)
+    given = (logits, ids, teacher) if weight is None else (logits, ids, teacher, weight)
+    dev = _device(*given, differentiable=logits)
     (logits, n, rows, stride), (ids, _, top, ids_stride), (teacher, _, _, teacher_stride) = _lists(logits, ids, teacher, "distill_loss_and_grad")
     if weight is not None:
         weight = _scales(weight, n, "distill_loss_and_grad")

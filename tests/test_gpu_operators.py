@@ -548,3 +548,34 @@ def test_refusals(cp, torch):
             call()
             pytest.fail("call %d was not refused" % k)
     cp.check_operator_status()
+
+
+def test_tensors_that_require_a_gradient(cp, torch):
+    """No graph is recorded, so a result that would be cut off from a tensor that wants a gradient is refused, not given."""
+    f = torch.randn((4, 8), device="cuda", requires_grad=True)
+    g = torch.randn((4, 8), device="cuda")
+    i8 = torch.ones((4, 8), dtype=torch.int8, device="cuda")
+    one, wanted = torch.ones(4, device="cuda"), torch.ones(4, device="cuda", requires_grad=True)
+    ids = torch.arange(4, device="cuda")
+    lists = torch.zeros((4, 2), dtype=torch.int64, device="cuda")
+    teacher, learned = torch.zeros((4, 2), device="cuda"), torch.zeros((4, 2), device="cuda", requires_grad=True)
+    calls = [
+        lambda: cp.embedding_lookup(f, ids), lambda: cp.embedding_lookup(f * 2, ids), lambda: cp.embedding_grad(ids, f, 4), lambda: cp.quantize_rows(f),
+        lambda: cp.int8_matmul(i8, wanted, i8, one), lambda: cp.int8_matmul(i8, one, i8, wanted), lambda: cp.distill_loss(f, lists, teacher),
+        lambda: cp.distill_loss(g, lists, learned), lambda: cp.distill_loss_and_grad(g, lists, learned), lambda: cp.distill_loss_and_grad(f, lists, learned),
+        lambda: cp.distill_loss_and_grad(f, lists, teacher, wanted),
+    ]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+            pytest.fail("call %d was not refused" % k)
+        with torch.no_grad():
+            call()
+    # the logits' gradient is what this call returns: it goes on from there
+    base = torch.randn((30, 8), device="cuda")
+    loss, grad = cp.distill_loss_and_grad(f @ base.T, lists, teacher)
+    assert not loss.requires_grad and not grad.requires_grad
+    logits = f @ base.T
+    logits.backward(cp.distill_loss_and_grad(logits, lists, teacher)[1])
+    assert torch.equal(f.grad, grad @ base)
+    assert torch.equal(cp.embedding_lookup(f.detach(), ids), f.detach())
