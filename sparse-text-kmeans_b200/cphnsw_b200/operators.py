@@ -10,9 +10,10 @@ workspace from torch's allocator; a tensor that another stream has written or wi
 with torch's own operations.  No autograd graph is recorded: the gradients are calls of their own.  While gradients are
 recorded a tensor that requires one is therefore refused (``detach()`` it, or call under ``torch.no_grad()``), except as
 the logits of ``distill_loss_and_grad``, whose gradient that call returns (``logits.backward(grad)`` goes on from
-there).  Matrices may have any row stride (0 for a broadcast row); where the elements of a row are not next to one
-another a contiguous copy is made.  Wrong arguments raise ``ValueError`` before anything is launched.
-``check_operator_status`` waits for the device and raises if a kernel gave up a bounded wait.
+there).  A tensor given as ``out`` counts as changed in place.  Matrices may have any row stride (0 for a broadcast
+row); where the elements of a row are not next to one another a contiguous copy is made.  Wrong arguments raise
+``ValueError`` before anything is launched.  ``check_operator_status`` waits for the device and raises if a kernel gave
+up a bounded wait.
 """
 import ctypes as C
 
@@ -22,11 +23,12 @@ _torch = None
 _fn = {}      # the library's functions, by their names without prefix
 _raw_stream = None
 _current_device = None
+_changed = None  # of a tensor: its values are others than autograd may have kept
 
 
 def _bind():
     """Loads torch and the library once; with argument types set, plain integers can be passed."""
-    global _torch, _raw_stream, _current_device
+    global _torch, _raw_stream, _current_device, _changed
     import torch
 
     from . import load_library
@@ -52,6 +54,7 @@ def _bind():
     # (the stream's address without a Stream object around it, which takes 2 us to make)
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
     _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    _changed = torch.autograd.graph.increment_version
     _torch = torch
 
 
@@ -100,12 +103,15 @@ def _matrix(t, what, dtypes=None):
     return t, n, d, stride if n > 1 else d or 1
 
 
-def _output(out, shape, dtype, dev, what):
-    """The caller's output, after a look at it."""
+def _output(out, shape, dtype, dev, what, replaced=None):
+    """The caller's output, after a look at it.  One that requires a gradient cannot be written to while gradients are recorded,
+    unless it is ``replaced``, and no leaf."""
     if not isinstance(out, _torch.Tensor) or not out.is_cuda or out.get_device() != dev or tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError("%s: out must be %s of shape %s on the inputs' device" % (what, dtype, tuple(shape)))
     if shape[-1] > 1 and out.stride(-1) != 1:
         raise ValueError("%s: out needs elements of a row next to one another" % what)
+    if out.requires_grad and _torch.is_grad_enabled() and (out is not replaced or out.is_leaf):
+        raise ValueError("%s: out requires a gradient" % what)
     return out
 
 
@@ -137,14 +143,17 @@ def embedding_lookup(table, ids, scale=1.0, out=None):
     ids = _flat_ids(ids, "embedding_lookup")
     n = ids.numel()
     shape = (*ids.shape, dim)
-    if out is None:
-        out = table.new_empty(shape)
-        stride = dim
-    else:
+    given = out is not None
+    if given:
         _output(out, shape, table.dtype, dev, "embedding_lookup")
         stride = _stride(out if out.dim() == 2 else out.view(n, dim))
+    else:
+        out = table.new_empty(shape)
+        stride = dim
     _call(dev, "embedding_lookup_dev", table.data_ptr(), _TYPES[table.dtype], rows, dim, table_stride, ids.data_ptr(), _IDS[ids.dtype], n, scale,
           out.data_ptr(), stride)
+    if given:
+        _changed(out)
     return out
 
 
@@ -168,10 +177,13 @@ def embedding_grad(ids, grad, rows, scale=1.0, dtype=None, out=None, accumulate=
     rows = int(rows)
     if rows < 1:
         raise ValueError("embedding_grad: need rows >= 1")
-    out = grad.new_empty((rows, dim), dtype=dtype) if out is None else _output(out, (rows, dim), dtype, dev, "embedding_grad")
+    given = out is not None
+    out = _output(out, (rows, dim), dtype, dev, "embedding_grad") if given else grad.new_empty((rows, dim), dtype=dtype)
     ws = _workspace(_fn["embedding_grad_workspace"](n, rows, dim), grad)
     _call(dev, "embedding_grad_dev", ids.data_ptr(), _IDS[ids.dtype], n, grad.data_ptr(), _TYPES[grad.dtype], grad_stride, scale, out.data_ptr(),
           _TYPES[dtype], rows, dim, _stride(out), int(bool(accumulate)), _ptr(ws), 0 if ws is None else ws.numel())
+    if given:
+        _changed(out)
     return out
 
 
@@ -209,16 +221,19 @@ def int8_matmul(a, a_scale, b, b_scale, dtype=None, out=None):
         dtype = _torch.bfloat16 if out is None else out.dtype
     if dtype not in _TYPES:
         raise ValueError("int8_matmul: element type %s is not supported" % dtype)
-    if out is None:
-        out, stride = a.new_empty((m, n), dtype=dtype), n or 1
-    else:
+    given = out is not None
+    if given:
         stride = _stride(_output(out, (m, n), dtype, dev, "int8_matmul"))
+    else:
+        out, stride = a.new_empty((m, n), dtype=dtype), n or 1
     pa, pb = a.data_ptr(), b.data_ptr()
     ws = None
     if (pa | pb | sa | sb) % 16:
         ws = _workspace(_fn["int8_matmul_workspace"](pa, sa, m, pb, sb, n, k), a)
     _call(dev, "int8_matmul_dev", pa, sa, a_scale.data_ptr(), m, pb, sb, b_scale.data_ptr(), n, k, out.data_ptr(), _TYPES[dtype], stride,
           _ptr(ws), 0 if ws is None else ws.numel())
+    if given:
+        _changed(out)
     return out
 
 
@@ -247,21 +262,24 @@ def distill_loss(logits, ids, teacher, temperature=1.0):
 def distill_loss_and_grad(logits, ids, teacher, weight=None, temperature=1.0, out=None):
     """``distill_loss`` and the gradient of its sum, weighted by ``weight`` float32 [n] (1 unless given), with respect to the
     logits, in their type: (loss [n], grad [n, rows]).  ``out`` may be ``logits`` itself."""
-    given = (logits, ids, teacher) if weight is None else (logits, ids, teacher, weight)
-    dev = _device(*given, differentiable=logits)
+    student = logits
+    tensors = (logits, ids, teacher) if weight is None else (logits, ids, teacher, weight)
+    dev = _device(*tensors, differentiable=student)
     (logits, n, rows, stride), (ids, _, top, ids_stride), (teacher, _, _, teacher_stride) = _lists(logits, ids, teacher, "distill_loss_and_grad")
     if weight is not None:
         weight = _scales(weight, n, "distill_loss_and_grad")
     if out is None:
         grad, grad_stride = logits.new_empty((n, rows)), rows or 1
     else:
-        grad = _output(out, (n, rows), logits.dtype, dev, "distill_loss_and_grad")
+        grad = _output(out, (n, rows), logits.dtype, dev, "distill_loss_and_grad", replaced=student)
         grad_stride = _stride(grad)
     loss = teacher.new_empty(n)
     ws = _workspace(_fn["distill_workspace"](n, top), teacher)
     _call(dev, "distill_loss_and_grad_dev", logits.data_ptr(), _TYPES[logits.dtype], n, rows, stride, ids.data_ptr(), _IDS[ids.dtype],
           ids_stride, teacher.data_ptr(), teacher_stride, top, temperature, _ptr(weight), loss.data_ptr(), grad.data_ptr(), grad_stride,
           _ptr(ws), 0 if ws is None else ws.numel())
+    if out is not None:
+        _changed(out)
     return loss, grad
 
 

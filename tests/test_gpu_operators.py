@@ -579,3 +579,40 @@ def test_tensors_that_require_a_gradient(cp, torch):
     logits.backward(cp.distill_loss_and_grad(logits, lists, teacher)[1])
     assert torch.equal(f.grad, grad @ base)
     assert torch.equal(cp.embedding_lookup(f.detach(), ids), f.detach())
+
+
+def test_outputs_count_as_changed(cp, torch):
+    """What is written to a caller's tensor autograd hears of, as of torch's own operations in place: a graph that had kept its
+    values refuses to go back through them, instead of going with others."""
+    f = torch.randn((4, 8), device="cuda", requires_grad=True)
+    lists, teacher = torch.zeros((4, 2), dtype=torch.int64, device="cuda"), torch.zeros((4, 2), device="cuda")
+    base = torch.randn((30, 8), device="cuda")
+    i8, one, ids = torch.ones((4, 8), dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"), torch.arange(4, device="cuda")
+    for given in (lambda t: t, lambda t: t.detach()):
+        logits = torch.exp(f @ base.T)  # (its derivative is its result)
+        _, grad = cp.distill_loss_and_grad(given(logits), lists, teacher, out=given(logits))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            logits.backward(grad)
+    # a graph that has not kept them goes on
+    want = cp.distill_loss_and_grad((f @ base.T).detach(), lists, teacher)[1] @ base
+    logits = f @ base.T
+    logits.backward(cp.distill_loss_and_grad(logits, lists, teacher, out=logits)[1])
+    assert torch.equal(f.grad, want)
+    table, grad = torch.randn((4, 8), device="cuda"), torch.randn((4, 8), device="cuda")
+    for write in (lambda out: cp.embedding_lookup(table, ids, out=out), lambda out: cp.embedding_grad(ids, grad, 4, out=out),
+                  lambda out: cp.embedding_grad(ids, grad, 4, out=out, accumulate=True), lambda out: cp.distill_loss_and_grad(grad, lists, teacher, out=out)):
+        out = torch.zeros((4, 8), device="cuda")
+        before = out._version
+        write(out)
+        assert out._version > before
+        with pytest.raises(ValueError, match="requires a gradient"):
+            write(f)  # (a leaf: torch does not change one in place either)
+        with pytest.raises(ValueError, match="requires a gradient"):
+            write(f * 2)
+    out = torch.zeros((4, 4), device="cuda")
+    before = out._version
+    cp.int8_matmul(i8, one, i8, one, out=out)
+    assert out._version > before
+    with torch.inference_mode():  # (tensors without a count)
+        out = torch.zeros((4, 8), device="cuda")
+        assert torch.equal(cp.embedding_lookup(table, ids, out=out), table)
