@@ -146,7 +146,10 @@ def embedding_lookup(table, ids, scale=1.0, out=None):
     given = out is not None
     if given:
         _output(out, shape, table.dtype, dev, "embedding_lookup")
-        stride = _stride(out if out.dim() == 2 else out.view(n, dim))
+        try:
+            stride = _stride(out if out.dim() == 2 else out.view(n, dim))
+        except RuntimeError:
+            raise ValueError("embedding_lookup: out needs rows at one distance from one another") from None
     else:
         out = table.new_empty(shape)
         stride = dim

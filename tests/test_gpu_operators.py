@@ -616,3 +616,15 @@ def test_outputs_count_as_changed(cp, torch):
     with torch.inference_mode():  # (tensors without a count)
         out = torch.zeros((4, 8), device="cuda")
         assert torch.equal(cp.embedding_lookup(table, ids, out=out), table)
+
+
+def test_lookup_into_rows_at_several_distances(cp, torch):
+    """Rows of `out` lie at one distance from one another; where they do not, it is refused like other wrong arguments."""
+    table, ids = torch.randn((50, 24), device="cuda"), torch.arange(15, device="cuda").view(3, 5)
+    room = torch.zeros((3, 5, 31), device="cuda")
+    cp.embedding_lookup(table, ids, out=room[:, :, 2:26])
+    assert torch.equal(room[:, :, 2:26], table[ids]) and not bool(room[:, :, :2].any()) and not bool(room[:, :, 26:].any())
+    room = torch.zeros((3, 7, 24), device="cuda")
+    with pytest.raises(ValueError, match="one distance"):
+        cp.embedding_lookup(table, ids, out=room[:, :5])
+    assert not bool(room.any())
