@@ -218,6 +218,37 @@ def test_grad_of_many_places(cp, torch, n, rows, dim):
     within(torch, cp.embedding_grad(ids, grad, rows, 0.5), want, size * EPS * (many + 2))
 
 
+# places of each id, in the order of the ids, by which runs begin and end inside pieces of 32, on their edges, and in the piece where
+# the one before ended; 8,193 places and more are over 256 pieces, and so joined three times
+LONG_RUNS = {
+    "inside": [20, 8295, 40, 33, 8200, 31, 32, 1, 64, 65, 500, 0, 17, 9000, 3],
+    "edges": [32, 8192, 64, 8224, 33, 31, 32, 96, 16_384, 0, 512, 544, 7],
+    "longest": [5, 300_007, 13, 50, 270_000, 2, 1000],
+    "one": [0, 2_200_000, 0],
+}
+
+
+@pytest.mark.parametrize("types", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp32")])
+@pytest.mark.parametrize("lengths,dim", [("inside", 3), ("inside", 264), ("inside", 1024), ("edges", 40), ("edges", 262), ("longest", 8), ("longest", 72), ("one", 4)])
+def test_grad_of_long_runs_exactly(cp, torch, types, lengths, dim):
+    """Whole numbers whose sums stay below 2^24: fp32 sums are exact in any order, so that a piece that is lost, counted twice or
+    joined to another run shows.  A tenth of the places name no row."""
+    gen = generator(torch, dim)
+    count = torch.tensor(LONG_RUNS[lengths], device="cuda")
+    ids = torch.repeat_interleave(torch.arange(len(count), device="cuda"), count)
+    ids = torch.cat([ids, torch.full((len(ids) // 10 + 2049,), -1, device="cuda")])
+    n, rows = len(ids), len(count)
+    ids = ids[torch.randperm(n, generator=gen, device="cuda")]
+    grad = torch.randint(-3, 8, (n, dim), generator=gen, device="cuda", dtype=torch.int8).to(dtype_of(torch, types[0]))
+    assert int(count.max()) * 7 < 2 ** 24
+    total = torch.stack([grad[ids == k].double().sum(0) for k in range(rows)])
+    for accumulate in (False, True):
+        out = torch.full((rows, dim), 3.0, dtype=dtype_of(torch, types[1]), device="cuda")
+        cp.embedding_grad(ids, grad, rows, 0.5, out=out, accumulate=accumulate)
+        want = (total * 0.5 + 3.0 * accumulate).to(out.dtype)
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("n,dim,dtype", [(5, 2049, "bf16"), (70, 2050, "fp32"), (33, 16_400, "bf16"), (9, 8196, "fp32"), (9, 8192, "fp32")])
 def test_quantize_rows_by_blocks(cp, torch, n, dim, dtype):
     gen = generator(torch, n + dim)
