@@ -6,6 +6,8 @@
 //   loss = T^2 sum_j p_j (log p_j - log q_{t_j}),   dz_v = weight T (q_v - sum over j with t_j = v of p_j).
 // A row whose list is empty (or all -inf) has loss 0 and gradient 0 whatever z holds; one whose logits are all -inf has
 // q = 0 throughout, and a loss of +inf.  Weight 0 gives a gradient of 0 whatever z holds.
+// A NaN or +inf among the logits makes the row's loss and all of its gradient NaN, a NaN among the list's the loss and the
+// gradient at the list's ids.
 //
 // Everything is computed in fp32: z_v is read as it is stored, q_v = 2^((z_v - m) c) / sum with c = log2(e) / T and m the
 // row's maximum, so that the size of the logits costs no precision; the gradient is rounded to the logits' type once.  A row's
@@ -239,7 +241,7 @@ __device__ __forceinline__ ListSums read_list(const Args& a, uint64_t row, const
         }
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            if (s[k] == -INFINITY) id[k] = kFull;  // (a NaN counts, and makes the row's results NaN)
+            if (s[k] == -INFINITY) id[k] = kFull;  // (a NaN counts: the loss is NaN, and the gradient at the list's ids)
             zj[k] = id[k] != kFull ? to_float(z[id[k]]) : 0.0f;
         }
 #pragma unroll

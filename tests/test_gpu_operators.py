@@ -478,6 +478,48 @@ def test_distill_of_masked_and_odd_rows(cp, torch):
     assert torch.equal(torch.isinf(cp.distill_loss(z, ids, teacher, 2.0)), torch.isinf(loss))
 
 
+# one length for each way a row can take: a warp (two sizes), small rings, large rings in one block and in clusters, pieces
+@pytest.mark.parametrize("name,rows", [("fp32", 40), ("bf16", 3001), ("fp32", 1500), ("bf16", 5003), ("fp32", 4000), ("fp16", 16_384), ("bf16", 100_003),
+                                       ("fp32", 300_001), ("fp32", 1_000_003), ("bf16", 1_200_005)])
+@pytest.mark.parametrize("layout", ["dense", "shifted"])
+def test_distill_of_odd_rows_by_sizes(cp, torch, name, rows, layout):
+    """Each kind of row by itself: what is not a number shows where the formula has it, and nowhere else."""
+    T = 2.0
+    base = torch.zeros((6, rows), device="cuda").to(dtype_of(torch, name))
+    place = rows - 7                     # (far from the list)
+    base[0] = -math.inf                  # nothing left of the student
+    base[1, place] = math.nan
+    base[2, place] = math.inf
+    base[3, 5] = -math.inf               # a candidate that the teacher wants and the student masks
+    ids = torch.tensor([[5, 6]] * 6, device="cuda")
+    teacher = torch.zeros((6, 2), device="cuda")
+    teacher[4, 1] = math.nan
+    z = laid_out(torch, base, layout)
+    loss, grad = cp.distill_loss_and_grad(z, ids, teacher, temperature=T)
+    alone = cp.distill_loss(z, ids, teacher, T)
+    for each in (loss, alone):
+        assert float(each[0]) == math.inf and float(each[3]) == math.inf
+        assert bool(torch.isnan(each[[1, 2, 4]]).all()) and bool(torch.isfinite(each[5]))
+        # T^2 (log 1/2 + log rows): logits all alike
+        assert abs(float(each[5]) - T * T * (math.log(0.5) + math.log(rows))) <= T * T * (2.0 ** -16 + 10 * 2.0 ** -20)
+    assert bool(torch.isnan(grad[[1, 2]]).all())
+    there = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    there[5:7] = True
+    assert bool(torch.isnan(grad[4, there]).all())
+    want = torch.zeros((6, rows), dtype=torch.float64, device="cuda")   # T (q - p)
+    want[3] = T / (rows - 1)
+    want[3, 5] = 0.0
+    want[4:] = T / rows
+    for row in (0, 3, 5):
+        want[row, there] -= T * 0.5
+    fine = torch.ones((6, rows), dtype=torch.bool, device="cuda")
+    fine[1:3], fine[4, there] = False, False
+    bound = (want.abs() + T * 0.5 * there) * 2.0 ** -16 + want.abs() * ULP[name] + FLOOR[name] * (1 + T)
+    within(torch, grad[fine], want[fine], bound[fine])
+    assert not bool(grad[0, ~there].any())
+    cp.check_operator_status()
+
+
 @pytest.mark.parametrize("rows", [50, 9000])
 def test_distill_grad_against_differences(cp, torch, rows):
     gen = generator(torch, rows)
