@@ -478,6 +478,15 @@ def test_distill_of_masked_and_odd_rows(cp, torch):
     assert torch.equal(torch.isinf(cp.distill_loss(z, ids, teacher, 2.0)), torch.isinf(loss))
 
 
+@pytest.mark.parametrize("name,n,rows,top,T", [("fp32", 5, 1_000_003, 16, 1.0), ("fp32", 40, 1_000_003, 1024, 2.0), ("bf16", 20, 1_200_005, 64, 1.0),
+                                               ("fp16", 13, 2_000_000, 700, 1.0)])
+@pytest.mark.parametrize("layout", ["dense", "shifted"])
+def test_distill_by_several_pieces_a_block(cp, torch, name, n, rows, top, T, layout):
+    """Rows longer than a cluster holds go in pieces; here a block takes up to 17 of them, so that its ring goes round many times."""
+    test_distill(cp, torch, name, n, rows, top, T, layout)
+    cp.check_operator_status()
+
+
 # one length for each way a row can take: a warp (two sizes), small rings, large rings in one block and in clusters, pieces
 @pytest.mark.parametrize("name,rows", [("fp32", 40), ("bf16", 3001), ("fp32", 1500), ("bf16", 5003), ("fp32", 4000), ("fp16", 16_384), ("bf16", 100_003),
                                        ("fp32", 300_001), ("fp32", 1_000_003), ("bf16", 1_200_005)])
