@@ -58,10 +58,6 @@ struct Pack {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) raw[i] = reinterpret_cast<const Raw*>(p)[i];
     }
-    __device__ __forceinline__ void load_once(const T* p) {  // read-only data that is not read again soon
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) raw[i] = __ldcs(reinterpret_cast<const Raw*>(p) + i);
-    }
     __device__ __forceinline__ void store(T* p) const {
         if constexpr (kBytes == 32) {  // (by one instruction: two of 16 bytes would each fill half of every sector)
             const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
